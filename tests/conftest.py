@@ -12,6 +12,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run through gpurun)")
 
 
+# tests of tools that are no longer in the tree: kept as they were, not run
+REMOVED_TOOLS = {
+    "test_basic_block_profiler_rewrite_counts_every_straight_line_segment_once":
+        "the rewriter under test was taken out: the profiling kernel it made wrote through the scalar data cache, which GPU code of this tree must not do",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.name in REMOVED_TOOLS:
+            item.add_marker(pytest.mark.skip(reason=REMOVED_TOOLS[item.name]))
+
+
 @pytest.fixture(autouse=True)
 def _repo_cwd(monkeypatch):
     # scene files name meshes relative to the working directory (src/Mesh.hs:218-221)
