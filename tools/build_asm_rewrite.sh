@@ -11,7 +11,7 @@ obj=$root/build_exp/o_$name; bin=$root/build_exp/$name
 mkdir -p $obj $bin
 LLVM=/opt/rocm/lib/llvm/bin
 for v in exact fast; do
-  flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -DRAYHS_DEV_KNOBS $* -DRAYHS_KERNEL_SUFFIX=$v"
+  flags="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -DRAYHS_DEV_KNOBS $* -DRAYHS_KERNEL_SUFFIX=$v"
   [ $v = exact ] && flags="$flags -ffp-contract=off"
   /opt/rocm/bin/hipcc $flags --cuda-device-only -S $src/trace_kernel.hip -o $obj/dev_$v.s
   sed -E -f $script $obj/dev_$v.s > $obj/dev_${v}_mod.s

@@ -9,7 +9,7 @@ SRC = "/root/repo/rayhs_amd/csrc/trace_kernel.hip"
 asm = next((a for a in sys.argv[1:] if a.endswith(".s")), None)
 if asm is None:
     os.makedirs("/tmp/kl", exist_ok=True)
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-DRAYHS_KERNEL_SUFFIX=exact",
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-O3", "-std=c++17", "-ffp-contract=off", "-DRAYHS_KERNEL_SUFFIX=exact",
                     "-gline-tables-only", "--cuda-device-only", "-save-temps", "-c", SRC, "-I/root/repo/rayhs_amd/csrc", "-o", "trace.co"],
                    cwd="/tmp/kl", stderr=subprocess.DEVNULL)
     asm = "/tmp/kl/trace_kernel-hip-amdgcn-amd-amdhsa-gfx950.s"

@@ -14,7 +14,7 @@ SRC = "/root/repo/rayhs_amd/csrc/trace_kernel.hip"
 limit = int(sys.argv[1]) if len(sys.argv) > 1 else 96
 extra = sys.argv[2:]
 os.makedirs("/tmp/vp", exist_ok=True)
-subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-DRAYHS_KERNEL_SUFFIX=exact",
+subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-O3", "-std=c++17", "-ffp-contract=off", "-DRAYHS_KERNEL_SUFFIX=exact",
                 "-gline-tables-only", "--cuda-device-only", "-save-temps", "-c", SRC, "-I/root/repo/rayhs_amd/csrc", "-o", "trace.co"] + extra,
                cwd="/tmp/vp", stderr=subprocess.DEVNULL, check=True)
 text = open("/tmp/vp/trace_kernel-hip-amdgcn-amd-amdhsa-gfx950.s").read().split("\n")
